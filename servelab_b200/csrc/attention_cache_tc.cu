@@ -53,8 +53,9 @@ constexpr int Q_PANEL = BM * 128, KV_PANEL = BN * 128, KV_TILE = PANELS * KV_PAN
 constexpr int OFF_K = PANELS * Q_PANEL;
 constexpr int OFF_V = OFF_K + 2 * KV_TILE;
 constexpr int AHEAD = 8;                       // tiles whose rows and scales the scout may know
-constexpr int OFF_SCALE = OFF_V + 2 * KV_TILE;         // [AHEAD][2][BN] floats: keys', values'
-constexpr int OFF_ROW = OFF_SCALE + AHEAD * 2 * BN * 4;        // [AHEAD][BN] cache rows, -1: none
+constexpr int OFF_SCALE = OFF_V + 2 * KV_TILE;         // [AHEAD][SCALES][BN] floats: keys' scales, values', log2 of the values'
+constexpr int SCALES = 3;
+constexpr int OFF_ROW = OFF_SCALE + AHEAD * SCALES * BN * 4;   // [AHEAD][BN] cache rows, -1: none
 constexpr int OFF_LOG = OFF_ROW + AHEAD * BN * 4;      // [AHEAD] log2 of a power of two above a tile's value scales
 constexpr int OFF_BAR = OFF_LOG + AHEAD * 4;
 constexpr int OFF_TOP = OFF_BAR + 320;                 // the queries' largest magnitude, of each warp that stages them
@@ -211,8 +212,9 @@ __device__ __forceinline__ void all_exponentials(uint32_t s_col, float scale, co
         sums[r] = t.x + t.y;
     }
 }
-// The largest score of each row (a lane a row), times the keys' scales.
-template <bool CODES> __device__ __forceinline__ float row_maximum(uint32_t s_col, float scale, const float* kscale) {
+// The largest score of each row (a lane a row), with codes the largest sum of a key's score and log2 of its value's scale: of one
+// key, so that a large scale whose key has no weight leaves the others' bits alone.  klog: as kscale, of those logarithms.
+template <bool CODES> __device__ __forceinline__ float row_maximum(uint32_t s_col, float scale, const float* kscale, const float* klog) {
     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
     for (int quarter = 0; quarter < 4; ++quarter) {
@@ -221,12 +223,15 @@ template <bool CODES> __device__ __forceinline__ float row_maximum(uint32_t s_co
         wait_ld16(s);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            float2 k = make_float2(scale, scale);
-            if constexpr (CODES) k = *reinterpret_cast<const float2*>(kscale + 16 * quarter + 8 * i);
+            float2 k = make_float2(scale, scale), w = make_float2(0.f, 0.f);
+            if constexpr (CODES) {
+                k = *reinterpret_cast<const float2*>(kscale + 16 * quarter + 8 * i);
+                w = *reinterpret_cast<const float2*>(klog + 16 * quarter + 8 * i);
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int at = 8 * (r >> 1) + 4 * i + 2 * (r & 1);
-                m[r] = fmaxf(m[r], fmaxf(__uint_as_float(s[at]) * k.x, __uint_as_float(s[at + 1]) * k.y));
+                m[r] = fmaxf(m[r], fmaxf(fmaf(__uint_as_float(s[at]), k.x, w.x), fmaf(__uint_as_float(s[at + 1]), k.y, w.y)));
             }
         }
     }
@@ -500,12 +505,17 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                     if (!mbar_wait(q_full, 0)) { gave_up(0x402); return false; }
                     factor = a.scale * LOG2E * slb_codes::power(254 - query_field_of(smem));
                 }
+                int top = -100;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    scales[place * 2 * BN + lane + 32 * i] = ksc[i] * factor;
-                    scales[place * 2 * BN + BN + lane + 32 * i] = vsc[i] * slb_codes::VALUE_FACTOR;
+                    float* to = scales + place * SCALES * BN + lane + 32 * i;
+                    const int log = slb_codes::scale_log2(vsc[i]);
+                    to[0] = ksc[i] * factor;
+                    to[BN] = vsc[i] * slb_codes::VALUE_FACTOR;
+                    to[2 * BN] = (float)log;
+                    top = max(top, log);
                 }
-                const int top = __reduce_max_sync(0xffffffffu, max(slb_codes::scale_log2(vsc[0]), slb_codes::scale_log2(vsc[1])));
+                top = __reduce_max_sync(0xffffffffu, top);
                 if (lane == 0) scale_logs[place] = top;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&scaled[place]);
@@ -611,13 +621,15 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                 continue;
             }
             fence_after();
-            const float* kscale = scales + (j % AHEAD) * 2 * BN;
+            const float* kscale = scales + (j % AHEAD) * SCALES * BN;
             const float* vscale = kscale + BN;
+            const float* vlog = kscale + 2 * BN;
             const uint32_t s_col = tmem + lane_base + 64 * (j & 1);
             const int k0 = kbeg + j * BN;
             const bool open = __all_sync(0xffffffffu, k0 >= view.lo && k0 + BN - 1 <= row_hi && k0 + BN <= kend);
             // Where every key is seen the exponentials are taken against the reference as it is.  The maximum is looked for
-            // first only where a row has none yet, or where their sum says that one may be above 2^8.
+            // first only where a row has none yet, or where their sum says that one times its scale may be above 2^8 (as it may
+            // if that key has the tile's largest scale: the search then tells).
             float alpha = 1.f, sum = 0.f, sums[4] = {0.f, 0.f, 0.f, 0.f};
             auto raise = [&](float mt) {
                 if (mt > m_ref + RESCALE_THRESHOLD || (m_ref == -INFINITY && mt != -INFINITY)) {
@@ -627,7 +639,7 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
             };
             if (CODES && !mbar_spin(&scaled[j % AHEAD], (j / AHEAD) & 1)) { gave_up(0x304); ok = false; break; }
             if (open) {
-                const int top = CODES ? scale_logs[j % AHEAD] : 0;  // log2 of a power of two above the value scales that count
+                const int top = CODES ? scale_logs[j % AHEAD] : 0;  // log2 of a power of two above the tile's value scales
                 const float limit = slb_codes::power(127 + 8 - top);
                 const int frag = 2 * (lane & 3);
                 bool again = __any_sync(0xffffffffu, m_ref == -INFINITY);
@@ -635,7 +647,7 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
 #pragma unroll 1
                 for (int attempt = 0; attempt < 2; ++attempt) {
                     if (again) {
-                        raise(row_maximum<CODES>(s_col, scale, kscale + frag) + (float)top);
+                        raise(row_maximum<CODES>(s_col, scale, kscale + frag, vlog + frag));
                         rows_to_fragments(m_ref == -INFINITY ? 0.f : m_ref, ref);
                     }
                     all_exponentials<CODES>(s_col, scale, kscale + frag, vscale + frag, ref, p, sums);
@@ -651,7 +663,7 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                 uint32_t v[32];
                 // (in halves and rarely: short code rather than fast)
                 const unsigned long long seen = seen_keys(a, view, k0, kend, base, q0);
-                float mt = -INFINITY, best = 0.f;
+                float mt = -INFINITY;
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
                     const unsigned bits = (unsigned)(seen >> (32 * half));
@@ -660,18 +672,13 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         const float4 k = CODES ? *reinterpret_cast<const float4*>(kscale + 32 * half + i) : make_float4(scale, scale, scale, scale);
-                        const float4 w = CODES ? *reinterpret_cast<const float4*>(vscale + 32 * half + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        const float ks[4] = {k.x, k.y, k.z, k.w}, vs[4] = {w.x, w.y, w.z, w.w};
+                        const float4 w = CODES ? *reinterpret_cast<const float4*>(vlog + 32 * half + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        const float ks[4] = {k.x, k.y, k.z, k.w}, logs[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool sees = bits >> (i + e) & 1u;
-                            const float x = __uint_as_float(v[i + e]) * ks[e];
-                            mt = fmaxf(mt, sees ? x : -INFINITY);
-                            best = fmaxf(best, sees && vs[e] < INFINITY ? vs[e] : 0.f);
-                        }
+                        for (int e = 0; e < 4; ++e)
+                            mt = fmaxf(mt, bits >> (i + e) & 1u ? fmaf(__uint_as_float(v[i + e]), ks[e], logs[e]) : -INFINITY);
                     }
                 }
-                if (CODES) mt += (float)slb_codes::scale_log2(best * (1.f / slb_codes::VALUE_FACTOR));    // (of keys that the row sees)
                 raise(mt);
                 const float row_ref = m_ref == -INFINITY ? 0.f : m_ref;
                 rows_to_fragments(row_ref, ref);

@@ -1,0 +1,204 @@
+"""Each form of the attention over a cache by its name, at the inputs where its numbers can go wrong: value scales and
+queries of far magnitudes in one tile, windows, peaked scores, infinities and NaN beside finite rows.  The form is forced, so that
+small sizes reach the kernel for many rows; bounds are those of ``cache8_cases.bound``."""
+
+import math
+
+import pytest
+import torch
+
+import cache8_cases as C
+import test_gpu_cache8 as B
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+# (form, blocks that share the keys, units with one more, blocks of a cluster, rows a block)
+FORMS = {"tc": ("tc", 1, 0, 1, 0), "tc3": ("tc", 3, 0, 1, 0), "tc+": ("tc", 1, 3, 1, 0), "few8": ("few", 1, 0, 2, 8),
+         "few16": ("few", 2, 0, 4, 16), "plain": ("plain", 2, 0, 1, 0)}
+
+
+@pytest.fixture
+def force(monkeypatch):
+    """``force(name)``: attention runs in that form from here on; the returned list names the form of every call."""
+    def forced(name):
+        form, parts, more, cluster, block = FORMS[name]
+        calls = []
+
+        def plan(fast, kind, tokens, requests, group, num_kv_heads, head_dim, longest_q, longest):
+            assert fast or form == "plain"
+            calls.append(form)
+            if form == "tc":
+                tiles = tokens * group // 128 + requests
+                return form, tiles, parts, min(more, tiles * num_kv_heads), 1, 0
+            return form, -(-longest_q * group // (block or 8)), parts, 0, cluster, block
+
+        monkeypatch.setattr(B.K(), "cache_attention_plan", plan)
+        return calls
+    return forced
+
+
+def chain(s):
+    """A mask under which every token sees what it sees causally."""
+    words = max(1, -(-max(s["q_lens"]) // 32))
+    bits = [(2 << j) - 1 for n in s["q_lens"] for j in range(n)]
+    rows = [[b >> 32 * w & 0xFFFFFFFF for w in range(words)] for b in bits]
+    positions = [c - n + j for n, c in zip(s["q_lens"], s["ctxs"]) for j in range(n)]
+    rest = s["q"].shape[0] - len(bits)                     # (rows behind the last request's)
+    rows, positions = rows + [[0] * words] * rest, positions + [0] * rest
+    return C.i32([[w - (1 << 32) if w >> 31 else w for w in row] for row in rows], DEV), C.i32(positions, DEV), bits, positions
+
+
+def attend_and_check(s, window=0):
+    """Causal; a cache in the compute type by way of a mask that says the same."""
+    if s["kind"] == "plain":
+        mask, positions, bits, at = chain(s)
+        B.attend(s, window=window, mask=mask, positions=positions)
+        B.check(s, window=window, bits=bits, positions=at)
+    else:
+        B.attend(s, window=window)
+        B.check(s, window=window)
+
+
+def place(s, slot, request=0):
+    page, at = divmod(slot, s["page"])
+    return s["table"][request, page].item(), at
+
+
+def set_row(s, name, slot, code, scale):
+    """One cached row of all kv heads: every element the code of that number, and its scale."""
+    page, at = place(s, slot)
+    row = torch.full((s["kv"], s["dim"]), float(code), device=DEV).to(s[name].dtype)
+    s[name].view(torch.uint8)[page, :, at] = row.view(torch.uint8)
+    s[name + "s"][page, :, at] = scale
+
+
+def leaning(kind, dim, q_lens, ctxs, seed):
+    """A step whose queries have a common part along (1, .., 1), so that a key along it has about one score for all of them;
+    and the scale with which a key of largest codes has the score 1 (natural units) there."""
+    s = B.step("bfloat16", kind, 14, 2, dim, q_lens, ctxs, 16, seed=seed)
+    s["q"].copy_((0.1 * s["q"].float() + 1.0).to(torch.bfloat16))
+    return s, 1.0 / (dim * C.LARGEST[kind] * s["scale"])
+
+
+FAST = ["tc", "tc3", "tc+", "few8", "few16"]
+
+
+@pytest.mark.parametrize("form", FAST)
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("slot", [2, 130, 389, 393])
+def test_a_large_value_row_of_no_weight(force, form, kind, dim, slot):
+    """Its scale is 2^30 times the others', its weight 2^-60 of theirs: it adds 2^-30 and must cost the others nothing.  In the
+    first tile, in one that all rows see, and among the step's own tokens (389: before the first row's, 393: seen by some)."""
+    calls = force(form)
+    s, one = leaning(kind, dim, [9], [400], 41)
+    set_row(s, "k", slot, -C.LARGEST[kind], 60 * math.log(2) * one)
+    page, at = place(s, slot)
+    s["vs"][page, :, at] *= 2.0 ** 30
+    attend_and_check(s)
+    assert calls == [FORMS[form][0]]
+
+
+@pytest.mark.parametrize("form", FAST)
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("slot", [2, 130, 389, 393])
+def test_a_key_that_takes_all_weight_and_has_no_value(force, form, kind, dim, slot):
+    """A first token that all others look at, its value row zeros: the result is what the others add, 2^-40 of theirs."""
+    calls = force(form)
+    s, one = leaning(kind, dim, [9], [400], 42)
+    set_row(s, "k", slot, C.LARGEST[kind], 40 * math.log(2) * one)
+    set_row(s, "v", slot, 0, C.TINY)
+    attend_and_check(s)
+    assert calls == [FORMS[form][0]]
+
+
+@pytest.mark.parametrize("form", FAST)
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_value_scales_over_forty_powers_of_two(force, form, kind):
+    calls = force(form)
+    s = B.step("bfloat16", kind, 14, 2, 64, [19], [700], 16, seed=43)
+    s["vs"] *= torch.exp2(torch.randint(-20, 21, s["vs"].shape, generator=B.gen(44), device=DEV).float())
+    for factor in (1.0, 2.0 ** 80, 2.0 ** -90):
+        attend_and_check({**s, "vs": s["vs"] * factor})
+    for factor in (2.0 ** 60, 2.0 ** -60, 2.0 ** 120):
+        attend_and_check({**s, "q": (s["q"].float() * factor).to(torch.bfloat16), "ks": s["ks"] / factor})
+    assert set(calls) == {FORMS[form][0]}
+
+
+@pytest.mark.parametrize("form", FAST + ["plain"])
+@pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [0, 1, 20, 130])
+def test_portions_and_windows(force, form, kind, dim, window):
+    calls = force(form)
+    s = B.step("bfloat16", kind, 14, 2, dim, [5, 0, 33, 1, 70], [5, 0, 200, 77, 331], 16, seed=47, pad=1)
+    attend_and_check(s, window)
+    assert calls == [FORMS[form][0]]
+
+
+@pytest.mark.parametrize("form", FAST)
+@pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
+@pytest.mark.parametrize("page", [1, 5, 64])
+def test_pages_of_any_size(force, form, kind, page):
+    force(form)
+    attend_and_check(B.step("bfloat16", kind, 14, 2, 64, [21, 3], [200, 131], page, seed=48), 40)
+
+
+@pytest.mark.parametrize("form", FAST)
+@pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_peaked_scores(force, form, kind, dim):
+    """Scores of some tens: references move in most tiles."""
+    force(form)
+    attend_and_check(B.step("bfloat16", kind, 14, 2, dim, [30, 1], [901, 300], 16, seed=49, spread=6.0))
+
+
+def near(s, clean, rows, window=0, bits=None, positions=None):
+    """The results of those rows (boolean [tokens, heads]) of a step's only request within their bounds; ``clean``: the step whose
+    inputs they go by."""
+    n, c, heads, dim = s["q_lens"][0], s["ctxs"][0], s["heads"], s["dim"]
+    k, v = (C.rows_of(clean[x], clean[x + "s"], s["table"][0], s["page"], c) for x in ("k", "v"))
+    want, mag, dots = C.attention(clean["q"].view(n, heads, dim), k, v, C.visible(n, c, window, bits, positions), s["scale"],
+                                  heads // s["kv"])
+    far = (s["out"].view(n, heads, dim).to(torch.float64) - want).abs() - C.bound(want, mag, dots, c, dim, True, torch.bfloat16)
+    return bool((far[rows] <= 0).all())
+
+
+def but(tokens, *none):
+    rows = torch.ones(tokens, 14, dtype=torch.bool, device=DEV)
+    for t in none:
+        rows[t] = False
+    return rows
+
+
+@pytest.mark.parametrize("form", FAST + ["plain"])
+@pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_query_row_that_is_not_finite(force, form, kind, bad):
+    """Its own result is no number; the rows beside it are as without it."""
+    force(form)
+    s = B.step("bfloat16", kind, 14, 2, 64, [12], [300], 16, seed=51)
+    t = {**s, "q": s["q"].clone()}
+    t["q"].view(12, 14, 64)[4, 5, 17] = bad
+    if kind == "plain":
+        mask, positions, _, _ = chain(s)
+        B.attend(t, mask=mask, positions=positions)
+    else:
+        B.attend(t)
+    assert torch.isnan(t["out"].view(12, 14, 64)[4, 5].float()).all()
+    assert near(t, s, but(12, (4, 5)))
+
+
+@pytest.mark.parametrize("form", FAST + ["plain"])
+@pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
+def test_the_same_bits_every_time(force, form, kind):
+    force(form)
+    s = B.step("bfloat16", kind, 14, 2, 128, [40, 1], [1500, 700], 16, seed=53)
+    attend_and_check(s)
+    first = s["out"].clone()
+    for _ in range(5):
+        s["out"].fill_(3.0)
+        attend_and_check(s)
+        assert torch.equal(s["out"], first)
