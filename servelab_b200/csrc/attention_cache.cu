@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 2 : 1) few_rows_kern
     float4* from_o = reinterpret_cast<float4*>(reinterpret_cast<unsigned char*>(smem) + few_ring_bytes<KIND, NT>());   // [blocks][share]
     uint2* q_frag = reinterpret_cast<uint2*>(from_o + NR * D / 4);   // [NT][KSTEPS][32], NT > 1
     __shared__ float2 red_ml[FEW_WARPS][NR], from_ml[MAX_CLUSTER][NR];     // (reference, sum) of each row
+    __shared__ float lows[FEW_WARPS][NR];              // the second numbers of references (cache_codes.cuh), with `coarse`
     if (a.cluster > 1) cluster_arrive();               // (blocks send to one another: all must have begun)
     bool begun = a.cluster == 1;
     pdl_wait();
@@ -209,6 +210,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 2 : 1) few_rows_kern
             }
         }
         if (NT > 1) __syncthreads();
+        bool coarse = false;                           // some row of the warp has a reference of two numbers
         float m[NT][2], l[NT][2], acc[NT][F::MT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -270,7 +272,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 2 : 1) few_rows_kern
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[nt][e] *= ksc[e >> 1] * row_factor[nt][e & 1];
+                for (int e = 0; e < 4; ++e)            // (rounded here: the maximum and the exponents go by the same number)
+                    sc[nt][e] = __fmul_rn(sc[nt][e], ksc[e >> 1] * row_factor[nt][e & 1]);
             if (!open) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -294,21 +297,62 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 2 : 1) few_rows_kern
                     const float top = fmaxf(sc[nt][c] + lv[0], sc[nt][c + 2] + lv[1]);
                     over |= top > m[nt][c] + LAZY_LOG2;
                 }
-            if (__any_sync(0xffffffffu, over)) {
+            if (__any_sync(0xffffffffu, over) || (KIND != CACHE_PLAIN && coarse)) {
+                auto rescale = [&](int nt, int c, float alpha) {
+                    l[nt][c] *= alpha;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                    for (int i = 0; i < F::MT; ++i) { acc[nt][i][c] *= alpha; acc[nt][i][c + 2] *= alpha; }
+                };
+                if constexpr (KIND != CACHE_PLAIN) {
+                    bool big = false;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float top = fmaxf(sc[nt][c] + lv[0], sc[nt][c + 2] + lv[1]);
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        top = fmaxf(top, m[nt][c]);
-                        const float alpha = top == -INFINITY ? 1.f : fast_exp2(m[nt][c] - top);
-                        m[nt][c] = top;
-                        l[nt][c] *= alpha;
-#pragma unroll
-                        for (int i = 0; i < F::MT; ++i) { acc[nt][i][c] *= alpha; acc[nt][i][c + 2] *= alpha; }
+                        for (int e = 0; e < 4; ++e) big |= slb_codes::coarse_score(sc[nt][e]);
+                    if (__any_sync(0xffffffffu, big) && !coarse) {
+                        coarse = true;
+                        if (lane < NR) lows[warp][lane] = 0.f;
+                        __syncwarp();
                     }
+                }
+                if (KIND == CACHE_PLAIN || !coarse) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float top = fmaxf(sc[nt][c] + lv[0], sc[nt][c + 2] + lv[1]);
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            top = fmaxf(top, m[nt][c]);
+                            rescale(nt, c, top == -INFINITY ? 1.f : fast_exp2(m[nt][c] - top));
+                            m[nt][c] = top;
+                        }
+                } else {                               // (from then on with every slice: the scores become relative here)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float hi = fmaxf(sc[nt][c], sc[nt][c + 2]);
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                            hi = fmaxf(hi, m[nt][c]);
+                            const float from = hi == -INFINITY ? 0.f : hi;
+                            float& low_of = lows[warp][8 * nt + 2 * lt + c];
+                            const float old = m[nt][c] - from + low_of;
+                            float low = fmaxf(old, fmaxf(sc[nt][c] - from + lv[0], sc[nt][c + 2] - from + lv[1]));
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) low = fmaxf(low, __shfl_xor_sync(0xffffffffu, low, o));
+                            if (low != -INFINITY) {
+                                rescale(nt, c, fast_exp2(old - low));
+                                sc[nt][c] = sc[nt][c] - from - low;
+                                sc[nt][c + 2] = sc[nt][c + 2] - from - low;
+                                const bool two = slb_codes::coarse_score(from);
+                                m[nt][c] = two ? from : from + low;
+                                if (lg == 0) low_of = two ? low : 0.f;
+                            }
+                        }
+                    __syncwarp();
+                }
             }
             // ---- probabilities, times the values' scales, as the B operand of O^T
             unsigned pb[NT][2];
@@ -318,7 +362,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 2 : 1) few_rows_kern
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float ref = m[nt][e & 1];
-                    p[e] = fast_exp2(sc[nt][e] - (ref == -INFINITY ? 0.f : ref));
+                    p[e] = fast_exp2(sc[nt][e] - (ref == -INFINITY || (KIND != CACHE_PLAIN && coarse) ? 0.f : ref));
                     l[nt][e & 1] += p[e];
                     if constexpr (KIND != CACHE_PLAIN) p[e] = p[e] != 0.f ? p[e] * vsc[e >> 1] : 0.f;   // (a scale may be NaN)
                 }
@@ -375,6 +419,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 2 : 1) few_rows_kern
             for (int c = 0; c < 2; ++c) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
+                if (KIND != CACHE_PLAIN && coarse) l[nt][c] *= fast_exp2(lows[warp][8 * nt + 2 * lt + c]);
                 if (lg == 0) red_ml[warp][8 * nt + 2 * lt + c] = make_float2(m[nt][c], l[nt][c]);
             }
         __syncthreads();
@@ -389,6 +434,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 2 : 1) few_rows_kern
                 for (int w = 0; w < FEW_WARPS; ++w) top = fmaxf(top, red_ml[w][8 * nt + 2 * lt + c].x);
                 // (a row without a reference has seen nothing, sum 0, or nothing but NaN)
                 f[c] = (m[nt][c] == -INFINITY ? l[nt][c] * 0.f : fast_exp2(m[nt][c] - top)) * BACK;
+                if (KIND != CACHE_PLAIN && coarse) f[c] *= fast_exp2(lows[warp][8 * nt + 2 * lt + c]);
             }
 #pragma unroll
             for (int i = 0; i < F::MT; ++i)

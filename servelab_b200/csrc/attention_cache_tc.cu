@@ -62,6 +62,9 @@ constexpr int OFF_TOP = OFF_BAR + 320;                 // the queries' largest m
 constexpr size_t SMEM = OFF_TOP + 4 * MMA_WARP;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_THRESHOLD = 8.f;       // log2 of the largest probability tolerated
+// References up to here go with scores in one multiply-add.  It takes the product as it is and the reference as the product
+// that was rounded: an exponent is off by up to half a unit in the last place, 2^-5 here, but 128 and more from 2^31 on.
+constexpr float FUSED_REFERENCE = 1048576.f;
 
 __device__ __forceinline__ void gave_up(int code) {
     if ((threadIdx.x & 31) == 0) atomicCAS(&cache_tc_status, 0, code);
@@ -605,7 +608,8 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
         const RowView view = row_view(a, base, q0 + local, local);
         const int row_hi = view.bits != nullptr ? base - 1 : view.hi;     // every key up to here and from view.lo on is seen
         // A row's reference and the sum of its probabilities, of the latter what came from fragments by itself.
-        float m_ref = -INFINITY, l = 0.f, ref[4] = {0.f, 0.f, 0.f, 0.f}, l_frag[4] = {0.f, 0.f, 0.f, 0.f};
+        // m_low: the second number of a reference (cache_codes.cuh), 0 but for scores that reach 2^24.
+        float m_ref = -INFINITY, m_low = 0.f, l = 0.f, ref[4] = {0.f, 0.f, 0.f, 0.f}, l_frag[4] = {0.f, 0.f, 0.f, 0.f};
         bool ok = true;
         for (int j = 0; j < ntiles && ok; ++j) {
             if (!(live ? mbar_spin(&s_full[j & 1], (j >> 1) & 1) : mbar_wait(&s_full[j & 1], (j >> 1) & 1))) {
@@ -626,7 +630,8 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
             const float* vlog = kscale + 2 * BN;
             const uint32_t s_col = tmem + lane_base + 64 * (j & 1);
             const int k0 = kbeg + j * BN;
-            const bool open = __all_sync(0xffffffffu, k0 >= view.lo && k0 + BN - 1 <= row_hi && k0 + BN <= kend);
+            bool open = __all_sync(0xffffffffu, k0 >= view.lo && k0 + BN - 1 <= row_hi && k0 + BN <= kend &&
+                                                    (m_ref == -INFINITY || fabsf(m_ref) <= FUSED_REFERENCE));
             // Where every key is seen the exponentials are taken against the reference as it is.  The maximum is looked for
             // first only where a row has none yet, or where their sum says that one times its scale may be above 2^8 (as it may
             // if that key has the tile's largest scale: the search then tells).
@@ -647,7 +652,10 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
 #pragma unroll 1
                 for (int attempt = 0; attempt < 2; ++attempt) {
                     if (again) {
-                        raise(row_maximum<CODES>(s_col, scale, kscale + frag, vlog + frag));
+                        const float mt = row_maximum<CODES>(s_col, scale, kscale + frag, vlog + frag);
+                        open = __all_sync(0xffffffffu, mt == -INFINITY || fabsf(mt) <= FUSED_REFERENCE);
+                        if (!open) break;
+                        raise(mt);
                         rows_to_fragments(m_ref == -INFINITY ? 0.f : m_ref, ref);
                     }
                     all_exponentials<CODES>(s_col, scale, kscale + frag, vscale + frag, ref, p, sums);
@@ -657,13 +665,19 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                     if (!again) break;
                 }
                 // P: 64 numbers of 16 bits = 32 columns, over the first half of this tile's scores
-                store_pairs(s_col, p[0]);
-                store_pairs(s_col + (16u << 16), p[1]);
-            } else {
+                if (open) {
+                    store_pairs(s_col, p[0]);
+                    store_pairs(s_col + (16u << 16), p[1]);
+                }
+            }
+            if (!open) {
+                // (sums of an attempt that was given up do not count)
+                sums[0] = sums[1] = sums[2] = sums[3] = 0.f;
                 uint32_t v[32];
                 // (in halves and rarely: short code rather than fast)
                 const unsigned long long seen = seen_keys(a, view, k0, kend, base, q0);
-                float mt = -INFINITY;
+                // (scores are rounded before their reference is taken off: see FUSED_REFERENCE)
+                float mt = -INFINITY, ms = -INFINITY;
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
                     const unsigned bits = (unsigned)(seen >> (32 * half));
@@ -675,11 +689,36 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                         const float4 w = CODES ? *reinterpret_cast<const float4*>(vlog + 32 * half + i) : make_float4(0.f, 0.f, 0.f, 0.f);
                         const float ks[4] = {k.x, k.y, k.z, k.w}, logs[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            mt = fmaxf(mt, bits >> (i + e) & 1u ? fmaf(__uint_as_float(v[i + e]), ks[e], logs[e]) : -INFINITY);
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = bits >> (i + e) & 1u ? __fmul_rn(__uint_as_float(v[i + e]), ks[e]) : -INFINITY;
+                            ms = fmaxf(ms, x);
+                            if (CODES) mt = fmaxf(mt, x + logs[e]);
+                        }
                     }
                 }
-                raise(mt);
+                const bool coarse = CODES && (slb_codes::coarse_score(ms) || slb_codes::coarse_score(m_ref));
+                if (CODES && __any_sync(0xffffffffu, coarse)) {
+                    const float hi = fmaxf(ms, m_ref), old = (m_ref - hi) + m_low;
+                    float low = old;
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        const unsigned bits = (unsigned)(seen >> (32 * half));
+                        tmem_ld32(s_col + 32 * half, v);
+                        wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float x = __fmul_rn(__uint_as_float(v[i]), kscale[32 * half + i]) - hi + vlog[32 * half + i];
+                            low = fmaxf(low, bits >> i & 1u ? x : -INFINITY);
+                        }
+                    }
+                    if (coarse) {
+                        const bool still = slb_codes::coarse_score(hi);
+                        alpha = exp2f(old - low);
+                        m_ref = still ? hi : hi + low;
+                        m_low = still ? low : 0.f;
+                    }
+                }
+                if (!coarse) raise(CODES ? mt : ms);
                 const float row_ref = m_ref == -INFINITY ? 0.f : m_ref;
                 rows_to_fragments(row_ref, ref);
                 // (each half of P goes behind its scores)
@@ -697,8 +736,8 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                         float p[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float x = __uint_as_float(v[i + e]) * ks[e];
-                            p[e] = slb_softmax::fast_exp2((bits >> (i + e) & 1u ? x : -INFINITY) - row_ref);
+                            const float x = __fmul_rn(__uint_as_float(v[i + e]), ks[e]);
+                            p[e] = slb_softmax::fast_exp2((bits >> (i + e) & 1u ? x : -INFINITY) - row_ref - m_low);
                             sum += p[e];
                             if (CODES) p[e] = p[e] == 0.f ? 0.f : p[e] * vs[e];       // (a scale may be NaN)
                         }
@@ -749,8 +788,9 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
             l_frag[i] += __shfl_xor_sync(0xffffffffu, l_frag[i], 2);
         }
         l += fragments_to_rows(l_frag);
+        if (CODES && parts > 1) l *= exp2f(m_low);
         const int h = kvh * g + rho - local * g;
-        const float unscale = (parts > 1 ? 1.f : l != 0.f ? 1.f / l : 0.f) * (CODES ? 1.f / slb_codes::VALUE_FACTOR : 1.f);
+        const float unscale = (parts > 1 ? exp2f(m_low) : l != 0.f ? 1.f / l : 0.f) * (CODES ? 1.f / slb_codes::VALUE_FACTOR : 1.f);
         // A partial result is a tile's, columns in fours: [unit][part][D / 4][BM], and [unit][part][BM] (reference, sum).  A
         // block that gave up leaves NaN there.
         const size_t piece = (size_t)(tile * a.Hkv + kvh) * (a.parts + (a.more > 0 ? 1 : 0)) + part;

@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) plain_cache_attention_kernel
                 float kscale = a.scale * 1.4426950408889634f;
                 if constexpr (KIND != CACHE_PLAIN) { kscale *= a.ks[row]; vscale = a.vs[row]; }
 #pragma unroll
-                for (int r = 0; r < PA_ROWS; ++r) sc[r] *= kscale;
+                for (int r = 0; r < PA_ROWS; ++r) sc[r] = __fmul_rn(sc[r], kscale);   // (the maximum and the exponents go by this number)
             }
 #pragma unroll
             for (int r = 0; r < PA_ROWS; ++r) {

@@ -8,7 +8,8 @@
 //     s + log2(scale) of the keys that the row sees (lazily: by 2^8).  Then probability x scale x 2^7 is at most 2^15, keys
 //     whose contribution is down to 2^-21 of the largest keep all bits of a float16, and the sum of the probabilities,
 //     in float32, has the same reference and cancels it.  (A scale of less than 2^-100 counts as 2^-100 there, one of more
-//     than 2^110 as that.)
+//     than 2^110 as that.)  Where scores reach 2^24 a sum with them is off by any power of two: the reference is kept in two
+//     numbers there, the largest score and, relative to it, the largest score + log2(scale).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -60,6 +61,8 @@ __device__ __forceinline__ unsigned half_pair(float lo, float hi) {
 }
 
 constexpr float VALUE_FACTOR = 128.f;          // 2^7, see above
+// a score whose reference is kept in two numbers, see above (an infinity, whose row has no result, is none)
+__device__ __forceinline__ bool coarse_score(float x) { return fabsf(x) >= 16777216.f && fabsf(x) < INFINITY; }
 // log2 of a power of two above a value scale, as far as it counts (an infinity or NaN, whose results are none: 0)
 __device__ __forceinline__ int scale_log2(float scale) {
     const int e = __float_as_int(scale) >> 23 & 255;

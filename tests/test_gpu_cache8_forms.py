@@ -155,6 +155,41 @@ def test_peaked_scores(force, form, kind, dim):
     attend_and_check(B.step("bfloat16", kind, 14, 2, dim, [30, 1], [901, 300], 16, seed=49, spread=6.0))
 
 
+def one_takes_all(s, q):
+    """(tokens, heads) whose best key leads by more than scores may be off (twice (D + 3) 2^-24 of their products' magnitudes) and
+    30 besides, and the value of that key [tokens, heads, D]."""
+    n, c, heads, dim = s["q_lens"][0], s["ctxs"][0], s["heads"], s["dim"]
+    k, v = (C.rows_of(s[x], s[x + "s"], s["table"][0], s["page"], c).repeat_interleave(heads // s["kv"], 0) for x in ("k", "v"))
+    q = q.view(n, heads, dim).transpose(0, 1).to(torch.float64)
+    scores = (q @ k.transpose(1, 2) * s["scale"]).masked_fill(~C.visible(n, c).to(DEV), -math.inf)
+    off = 2 * (dim + 3) * 2.0 ** -24 * (q.abs() @ k.abs().transpose(1, 2) * s["scale"]).amax(-1)
+    best = scores.topk(2, -1)
+    value = torch.gather(v, 1, best.indices[..., :1].expand(-1, -1, dim))
+    return (best.values[..., 0] - best.values[..., 1] > 2 * off + 30).T, value.transpose(0, 1)
+
+
+@pytest.mark.parametrize("form", FAST + ["plain"])
+@pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("far", [18, 22, 24, 25, 26, 27, 28, 30, 34, 60])
+def test_scores_of_any_size(force, form, kind, dim, far):
+    """Scores of about 2^far, also where all of them are negative: numbers throughout, and one key's value where float32 tells
+    which; for value scales of different sizes."""
+    force(form)
+    s = B.step("bfloat16", kind, 14, 2, dim, [12], [300], 16, seed=54)
+    s["q"] = (2.0 ** far * s["q"].float()).to(torch.bfloat16)
+    below = {**s, "q": (s["q"].float().abs()).to(torch.bfloat16), "k": -s["k"].abs() if kind != "e4m3" else
+             (s["k"].view(torch.uint8) | 0x80).view(s["k"].dtype)}
+    for t in (s, below):
+        for factor in (1.0,) if kind == "plain" else (1.0, 2.0 ** -20, 2.0 ** 10):
+            u = {**t, "vs": None if kind == "plain" else t["vs"] * factor}
+            attend_and_check(u)
+            sure, value = one_takes_all(u, u["q"])
+            assert sure.float().mean() > 0.75
+            off = (u["out"].view(12, 14, dim).to(torch.float64) - value).abs()[sure]
+            assert (off <= 2.0 ** -7 * value[sure].abs() + 1e-30).all()
+
+
 def near(s, clean, rows, window=0, bits=None, positions=None):
     """The results of those rows (boolean [tokens, heads]) of a step's only request within their bounds; ``clean``: the step whose
     inputs they go by."""
