@@ -58,8 +58,10 @@ constexpr int SCALES = 3;
 constexpr int OFF_ROW = OFF_SCALE + AHEAD * SCALES * BN * 4;   // [AHEAD][BN] cache rows, -1: none
 constexpr int OFF_LOG = OFF_ROW + AHEAD * BN * 4;      // [AHEAD] log2 of a power of two above a tile's value scales
 constexpr int OFF_BAR = OFF_LOG + AHEAD * 4;
-constexpr int OFF_TOP = OFF_BAR + 320;                 // the queries' largest magnitude, of each warp that stages them
-constexpr size_t SMEM = OFF_TOP + 4 * MMA_WARP;
+constexpr int OFF_TOP = OFF_BAR + 320;                 // [BM] largest magnitude of each row of the queries, 16 bits
+constexpr int OFF_SPREAD = OFF_TOP + 2 * BM;           // [MMA_WARP] largest and least of what a warp stages, 16 bits each
+constexpr int OFF_FIELD = OFF_SPREAD + 4 * MMA_WARP;   // the queries' factor
+constexpr size_t SMEM = OFF_FIELD + 16;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_THRESHOLD = 8.f;       // log2 of the largest probability tolerated
 // References up to here go with scores in one multiply-add.  It takes the product as it is and the reference as the product
@@ -245,10 +247,25 @@ template <bool CODES> __device__ __forceinline__ float row_maximum(uint32_t s_co
     }
     return fragments_to_rows(m);
 }
-// the exponent field of the tile's queries' factor, behind their barrier
-__device__ __forceinline__ int query_field_of(const unsigned char* smem) {
-    const uint4 a = *reinterpret_cast<const uint4*>(smem + OFF_TOP), b = *reinterpret_cast<const uint4*>(smem + OFF_TOP + 16);
-    return slb_codes::query_field(__uint_as_float(max(max(max(a.x, a.y), max(a.z, a.w)), max(max(b.x, b.y), max(b.z, b.w))) << 16));
+// Powers of two that bring the tile's queries into float16, as exponent fields.  One for all rows (`field`) where each row's
+// largest element lies within 2^16 of the tile's: then an element is off by at most 2^-22 of its row's largest.  Otherwise
+// (`wide`) a row has its own, at most 2^126 above the tile's.
+struct QueryFactors {
+    int field;
+    bool wide;
+};
+// 16-bit magnitudes: the largest, and one less than the least that is not zero
+struct Spread {
+    unsigned top, least;
+    __device__ __forceinline__ bool wide() const { return least != 0xffffu && (int)(top >> 7) - (int)((least + 1) >> 7) > 16; }
+};
+__device__ __forceinline__ Spread spread_of(unsigned tops, unsigned leasts) {      // of pairs, over a warp
+    return {__reduce_max_sync(0xffffffffu, max(tops & 0xffffu, tops >> 16)), __reduce_min_sync(0xffffffffu, min(leasts & 0xffffu, leasts >> 16))};
+}
+__device__ __forceinline__ int row_field(const unsigned char* smem, int row, const QueryFactors& f) {
+    if (!f.wide) return f.field;
+    const unsigned top = reinterpret_cast<const unsigned short*>(smem + OFF_TOP)[row];
+    return min(slb_codes::query_field(__uint_as_float(top << 16)), f.field + 126);
 }
 
 // grid: units of 128 rows and kv head, each with its shares of the keys
@@ -347,8 +364,7 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
 
     if (warp < MMA_WARP) {
         // Queries: softmax and loader warps (whose rows are being looked up) stage 16 rows each, D / 8 lanes a row.  With codes
-        // the queries of the whole tile become float16 with one power of two: an element is off by at most 2^-38 of the
-        // tile's largest, so its scores by as much of that row's.
+        // they become float16 by powers of two (QueryFactors).
         constexpr int LANES = D / 8, AT_ONCE = 32 / LANES, MINE = BM / MMA_WARP, ROUNDS = MINE / AT_ONCE;
         const int c = lane % LANES, rho = row0 + min(MINE * warp + lane % MINE, nrows - 1), local = rho / g;
         const bf16* mine = reinterpret_cast<const bf16*>(a.q) + (size_t)(q0 + local) * a.ldq + (size_t)(kvh * g + rho - local * g) * D;
@@ -358,39 +374,54 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
             const unsigned long long row = __shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)mine, i * AT_ONCE + lane / LANES);
             x[i] = reinterpret_cast<const uint4*>((uintptr_t)row)[c];
         }
-        float factor = 1.f;
+        QueryFactors factors = {};
         if constexpr (CODES) {
-            unsigned lo = 0, hi = 0;                        // largest magnitudes, bfloat16 bits
+            // Of every 16 bytes the largest magnitude (bfloat16 bits), in pairs of rounds: if those lie near enough to one another,
+            // rows do.
+            unsigned tops[ROUNDS / 2], most = 0, leasts = 0xffffffffu;
 #pragma unroll
             for (int i = 0; i < ROUNDS; ++i) {
-                const unsigned w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                const unsigned both = __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu), __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
+                const unsigned top = max(both & 0xffffu, both >> 16);
+                tops[i / 2] = i % 2 ? tops[i / 2] | top << 16 : top;
+            }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    lo = max(lo, w[e] & 0x7fffu);
-                    hi = max(hi, w[e] & 0x7fff0000u);
-                }
+            for (int i = 0; i < ROUNDS / 2; ++i) {
+                most = __vmaxu2(most, tops[i]);
+                leasts = __vminu2(leasts, __vsub2(tops[i], 0x00010001u));
             }
-            unsigned top = __reduce_max_sync(0xffffffffu, max(lo, hi >> 16));
-            if (top >= 0x7f80u) {                           // infinities and NaN do not count (their rows have no result)
-                top = 0;
-#pragma unroll 1
-                for (int i = 0; i < MINE * D / 2; i += 32) {
-                    const unsigned w = *reinterpret_cast<const unsigned*>(
-                        (uintptr_t)__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)mine, i / (D / 2)) + 4 * ((i + lane) % (D / 2)));
-                    if ((w & 0x7fffu) < 0x7f80u) top = max(top, w & 0x7fffu);
-                    if ((w >> 16 & 0x7fffu) < 0x7f80u) top = max(top, w >> 16 & 0x7fffu);
-                }
-                top = __reduce_max_sync(0xffffffffu, top);
-            }
-            if (lane == 0) reinterpret_cast<unsigned*>(smem + OFF_TOP)[warp] = top;
+            Spread s = spread_of(most, leasts);
+            if (lane == 0) reinterpret_cast<unsigned*>(smem + OFF_SPREAD)[warp] = s.top | s.least << 16;
             asm volatile("bar.sync 1, %0;" ::"n"(32 * MMA_WARP) : "memory");
-            factor = slb_codes::power(query_field_of(smem));
+            const uint4 u = *reinterpret_cast<const uint4*>(smem + OFF_SPREAD), w = *reinterpret_cast<const uint4*>(smem + OFF_SPREAD + 16);
+            s.top = __vmaxu2(__vmaxu2(__vmaxu2(u.x, u.y), __vmaxu2(u.z, u.w)), __vmaxu2(__vmaxu2(w.x, w.y), __vmaxu2(w.z, w.w))) & 0xffffu;
+            s.least = __vminu2(__vminu2(__vminu2(u.x, u.y), __vminu2(u.z, u.w)), __vminu2(__vminu2(w.x, w.y), __vminu2(w.z, w.w))) >> 16;
+            if (s.wide() || s.top >= 0x7f80u) {             // (in all of these warps) row by row
+#pragma unroll
+                for (int i = 0; i < ROUNDS; i += 2) {
+                    unsigned rows = tops[i / 2];
+#pragma unroll
+                    for (int o = LANES / 2; o > 0; o >>= 1) rows = __vmaxu2(rows, __shfl_xor_sync(0xffffffffu, rows, o));
+                    if (c < 2) {                            // (a row with an infinity or NaN does not count: it has no result)
+                        const unsigned top = c == 0 ? rows & 0xffffu : rows >> 16;
+                        reinterpret_cast<unsigned short*>(smem + OFF_TOP)[warp * MINE + (i + c) * AT_ONCE + lane / LANES] =
+                            (unsigned short)(top < 0x7f80u ? top : 0);
+                    }
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * MMA_WARP) : "memory");
+                const uint2 t4 = reinterpret_cast<const uint2*>(smem + OFF_TOP)[lane];
+                s = spread_of(__vmaxu2(t4.x, t4.y), __vminu2(__vsub2(t4.x, 0x00010001u), __vsub2(t4.y, 0x00010001u)));
+                factors.wide = s.wide();
+            }
+            factors.field = slb_codes::query_field(__uint_as_float(s.top << 16));
+            if (threadIdx.x == 0) *reinterpret_cast<QueryFactors*>(smem + OFF_FIELD) = factors;
         }
 #pragma unroll
         for (int i = 0; i < ROUNDS; ++i) {
             const int qr = warp * MINE + i * AT_ONCE + lane / LANES;
             uint4 y = x[i];
             if constexpr (CODES) {
+                const float factor = slb_codes::power(row_field(smem, qr, factors));
                 if (slb_codes::swaps<KIND>())
                     y = make_uint4(__byte_perm(y.x, y.y, 0x5410), __byte_perm(y.x, y.y, 0x7632),
                                    __byte_perm(y.z, y.w, 0x5410), __byte_perm(y.z, y.w, 0x7632));
@@ -506,7 +537,7 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                 const int place = j % AHEAD;
                 if (j == 0) {
                     if (!mbar_wait(q_full, 0)) { gave_up(0x402); return false; }
-                    factor = a.scale * LOG2E * slb_codes::power(254 - query_field_of(smem));
+                    factor = a.scale * LOG2E * slb_codes::power(254 - reinterpret_cast<const QueryFactors*>(smem + OFF_FIELD)->field);
                 }
                 int top = -100;
 #pragma unroll
@@ -606,7 +637,11 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
         const bool live = warp * 32 < nrows;                // (a warp whose rows are all padding only hands tiles on)
         const float scale = a.scale * LOG2E;                // (with codes it is in the keys' scales)
         const RowView view = row_view(a, base, q0 + local, local);
-        const int row_hi = view.bits != nullptr ? base - 1 : view.hi;     // every key up to here and from view.lo on is seen
+        int row_hi = view.bits != nullptr ? base - 1 : view.hi;           // every key up to here and from view.lo on is seen
+        if (CODES && ntiles > 0) {                          // (rows with factors of their own go the way of masked tiles)
+            if (!mbar_wait(q_full, 0)) gave_up(0x305);
+            if (reinterpret_cast<const QueryFactors*>(smem + OFF_FIELD)->wide) row_hi = -1;
+        }
         // A row's reference and the sum of its probabilities, of the latter what came from fragments by itself.
         // m_low: the second number of a reference (cache_codes.cuh), 0 but for scores that reach 2^24.
         float m_ref = -INFINITY, m_low = 0.f, l = 0.f, ref[4] = {0.f, 0.f, 0.f, 0.f}, l_frag[4] = {0.f, 0.f, 0.f, 0.f};
@@ -677,7 +712,11 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                 // (in halves and rarely: short code rather than fast)
                 const unsigned long long seen = seen_keys(a, view, k0, kend, base, q0);
                 // (scores are rounded before their reference is taken off: see FUSED_REFERENCE)
-                float mt = -INFINITY, ms = -INFINITY;
+                float mt = -INFINITY, ms = -INFINITY, row_scale = 1.f;
+                if constexpr (CODES) {                      // what the row's scores have besides the tile's factor
+                    const QueryFactors f = *reinterpret_cast<const QueryFactors*>(smem + OFF_FIELD);
+                    row_scale = slb_codes::power(127 + f.field - row_field(smem, r, f));
+                }
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
                     const unsigned bits = (unsigned)(seen >> (32 * half));
@@ -690,7 +729,7 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                         const float ks[4] = {k.x, k.y, k.z, k.w}, logs[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float x = bits >> (i + e) & 1u ? __fmul_rn(__uint_as_float(v[i + e]), ks[e]) : -INFINITY;
+                            const float x = bits >> (i + e) & 1u ? __fmul_rn(__uint_as_float(v[i + e]), ks[e] * row_scale) : -INFINITY;
                             ms = fmaxf(ms, x);
                             if (CODES) mt = fmaxf(mt, x + logs[e]);
                         }
@@ -707,7 +746,7 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                         wait_ld();
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            const float x = __fmul_rn(__uint_as_float(v[i]), kscale[32 * half + i]) - hi + vlog[32 * half + i];
+                            const float x = __fmul_rn(__uint_as_float(v[i]), kscale[32 * half + i] * row_scale) - hi + vlog[32 * half + i];
                             low = fmaxf(low, bits >> i & 1u ? x : -INFINITY);
                         }
                     }
@@ -736,7 +775,7 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                         float p[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float x = __fmul_rn(__uint_as_float(v[i + e]), ks[e]);
+                            const float x = __fmul_rn(__uint_as_float(v[i + e]), CODES ? ks[e] * row_scale : ks[e]);
                             p[e] = slb_softmax::fast_exp2((bits >> (i + e) & 1u ? x : -INFINITY) - row_ref - m_low);
                             sum += p[e];
                             if (CODES) p[e] = p[e] == 0.f ? 0.f : p[e] * vs[e];       // (a scale may be NaN)

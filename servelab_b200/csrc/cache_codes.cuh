@@ -2,8 +2,9 @@
 //
 // Both kinds become float16 (11 significant bits against 8 of an 8-bit integer and 4 of e4m3), which costs 5 instructions
 // for four int8 codes and 2 for four e4m3 codes (into bfloat16: 7 and 9).  float16's range needs two powers of two:
-//   * queries are scaled so that the largest element of a row (of a tile of rows in the tcgen05 kernel) lies in [2^13, 2^14):
-//     bfloat16 elements down to 2^-28 of it stay exact, what is smaller loses bits that the float32 sums do not have;
+//   * queries are scaled so that the largest element of a row (in the tcgen05 kernel of a tile of rows, as long as each row's
+//     lies within 2^16 of it) lies in [2^13, 2^14): bfloat16 elements down to 2^-28 of it stay exact, what is smaller loses bits
+//     that the float32 sums do not have;
 //   * a probability 2^(s - m) is taken against a reference m that counts value scales too: m follows the largest
 //     s + log2(scale) of the keys that the row sees (lazily: by 2^8).  Then probability x scale x 2^7 is at most 2^15, keys
 //     whose contribution is down to 2^-21 of the largest keep all bits of a float16, and the sum of the probabilities,

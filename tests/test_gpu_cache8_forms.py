@@ -190,6 +190,21 @@ def test_scores_of_any_size(force, form, kind, dim, far):
             assert (off <= 2.0 ** -7 * value[sure].abs() + 1e-30).all()
 
 
+@pytest.mark.parametrize("form", FAST)
+@pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("far", [14, 16, 17, 20, 34, 60, 100])
+def test_query_rows_of_very_different_size(force, form, kind, dim, far):
+    """Tokens and heads whose queries are 2^far times their neighbours', above or below."""
+    force(form)
+    s = B.step("bfloat16", kind, 14, 2, dim, [23], [300], 16, seed=50)
+    for heads in (slice(3, 14, 3), slice(1, 14, 2)):
+        q = s["q"].float().view(23, 14, dim).clone()
+        q[::2, heads] *= 2.0 ** far
+        attend_and_check({**s, "q": q.view(23, 14 * dim).to(torch.bfloat16)})
+        attend_and_check({**s, "q": (q.view(23, 14 * dim) * 2.0 ** -far).to(torch.bfloat16)})
+
+
 def near(s, clean, rows, window=0, bits=None, positions=None):
     """The results of those rows (boolean [tokens, heads]) of a step's only request within their bounds; ``clean``: the step whose
     inputs they go by."""
