@@ -228,13 +228,15 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 2 : 1) few_rows_kern
             const unsigned char* ks_at = ring + stage * F::SLICE;
             const unsigned char* vs_at = ks_at + KEYS * F::ROW_BYTES;
             stage = stage == F::STAGES - 1 ? 0 : stage + 1;
-            float ksc[2] = {1.f, 1.f}, vsc[2] = {1.f, 1.f};       // of keys lg and lg + 8
+            float ksc[2] = {1.f, 1.f}, vsc[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};      // of keys lg and lg + 8; log2 of the values'
             if constexpr (KIND != CACHE_PLAIN) {
                 const float* sc_at = reinterpret_cast<const float*>(vs_at + KEYS * F::ROW_BYTES);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     ksc[i] = sc_at[lg + 8 * i];
-                    vsc[i] = sc_at[16 + lg + 8 * i] * slb_codes::VALUE_FACTOR;
+                    vsc[i] = sc_at[16 + lg + 8 * i];
+                    lv[i] = (float)slb_codes::scale_log2(vsc[i]);
+                    vsc[i] *= slb_codes::VALUE_FACTOR;
                 }
             }
             // ---- scores of 16 keys
@@ -284,11 +286,6 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 2 : 1) few_rows_kern
                     }
             }
             // ---- the rows' references move rarely
-            float lv[2] = {0.f, 0.f};
-            if constexpr (KIND != CACHE_PLAIN) {
-                lv[0] = (float)(slb_codes::scale_log2(vsc[0]) - 7);
-                lv[1] = (float)(slb_codes::scale_log2(vsc[1]) - 7);
-            }
             bool over = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)

@@ -216,7 +216,8 @@ def cache8_attention(q, k_cache, v_cache, k_scale, v_scale, out, table, cu_q, ct
     s has the tokens ``cu_q[s]`` .. ``cu_q[s + 1]`` - 1, its newest cached ones of ``ctx_len[s]``.  ``longest_q`` and
     ``longest_context``: what the step's plan says of the most tokens and keys of a request; launch shapes go by them,
     results do not.  Rows behind the last request's are left as they are.  bfloat16 with head sizes 64 and 128 and rows of
-    whole 16-byte pieces: tensor cores; otherwise the plain kernel, float32 throughout."""
+    whole 16-byte pieces: tensor cores, for cached values of up to 2^117 (int8) or 2^118; otherwise the plain kernel, float32
+    throughout."""
     if k_scale is None or v_scale is None:
         raise L.KernelError("cache8_attention: an 8-bit cache needs its scales (tree_attention and paged_attention take others)")
     _cache_attention("cache8_attention", q, k_cache, v_cache, k_scale, v_scale, out, table, cu_q, ctx_len, None, None, H, Hkv, D,

@@ -127,6 +127,16 @@ def test_value_scales_over_forty_powers_of_two(force, form, kind):
     assert set(calls) == {FORMS[form][0]}
 
 
+@pytest.mark.parametrize("form", FAST)
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_value_scales_near_the_largest_that_count(force, form, kind):
+    """All scales from 2^104 to 2^110: values of up to 2^117 (int8) or 2^118."""
+    force(form)
+    s = B.step("bfloat16", kind, 14, 2, 64, [5], [300], 16, seed=45)
+    scale = torch.exp2(104 + 5.9 * torch.rand(s["vs"].shape, generator=B.gen(46), device=DEV))
+    attend_and_check({**s, "vs": torch.where(torch.isnan(s["vs"]), s["vs"], scale)})
+
+
 @pytest.mark.parametrize("form", FAST + ["plain"])
 @pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
 @pytest.mark.parametrize("dim", [64, 128])
