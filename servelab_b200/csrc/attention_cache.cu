@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, NT == 1 ? 2 : 1) few_rows_kern
                     const float ref = m[nt][e & 1];
                     p[e] = fast_exp2(sc[nt][e] - (ref == -INFINITY || (KIND != CACHE_PLAIN && coarse) ? 0.f : ref));
                     l[nt][e & 1] += p[e];
-                    if constexpr (KIND != CACHE_PLAIN) p[e] = p[e] != 0.f ? p[e] * vsc[e >> 1] : 0.f;   // (a scale may be NaN)
+                    if constexpr (KIND != CACHE_PLAIN) p[e] = sc[nt][e] != -INFINITY ? p[e] * vsc[e >> 1] : 0.f;   // (NaN counts where it is seen)
                 }
                 pb[nt][0] = movmatrix_trans(KIND == CACHE_PLAIN ? pack_bf16(p[0], p[1]) : slb_codes::half_pair(p[0], p[1]));
                 pb[nt][1] = movmatrix_trans(KIND == CACHE_PLAIN ? pack_bf16(p[2], p[3]) : slb_codes::half_pair(p[2], p[3]));

@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_tc_kernel(const Ca
                             const float x = __fmul_rn(__uint_as_float(v[i + e]), CODES ? ks[e] * row_scale : ks[e]);
                             p[e] = slb_softmax::fast_exp2((bits >> (i + e) & 1u ? x : -INFINITY) - row_ref - m_low);
                             sum += p[e];
-                            if (CODES) p[e] = p[e] == 0.f ? 0.f : p[e] * vs[e];       // (a scale may be NaN)
+                            if (CODES) p[e] = bits >> (i + e) & 1u ? p[e] * vs[e] : 0.f;      // (NaN counts where it is seen)
                         }
                         few[i >> 1] = CODES ? slb_codes::half_pair(p[0], p[1]) : slb_softmax::pack2(p[0], p[1]);
                         few[(i >> 1) + 1] = CODES ? slb_codes::half_pair(p[2], p[3]) : slb_softmax::pack2(p[2], p[3]);

@@ -252,6 +252,31 @@ def test_a_query_row_that_is_not_finite(force, form, kind, bad):
 
 
 @pytest.mark.parametrize("form", FAST + ["plain"])
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_scales_of_rows_that_are_not_seen(force, form, kind):
+    """NaN and infinite scales of a draft on another branch, of slots behind a causal token and before a window."""
+    force(form)
+    s = B.step("bfloat16", kind, 14, 2, 64, [6], [140], 16, seed=52)
+    page, at = place(s, 134 + 3)                           # drafted token 3: seen by itself alone
+    bits, where = [1, 3, 7, 15, 17, 49], list(range(134, 140))
+    for k_scale, v_scale in ((math.nan, math.inf), (math.inf, math.nan), (math.nan, 1.0), (1.0, math.nan)):
+        t = {**s, "ks": s["ks"].clone(), "vs": s["vs"].clone()}
+        t["ks"][page, :, at], t["vs"][page, :, at] = k_scale, v_scale
+        B.attend(t, mask=C.i32([[b] for b in bits], DEV), positions=C.i32(where, DEV))
+        assert near(t, s, but(6, 3), bits=bits, positions=where)
+        none = torch.isnan(t["out"][3].float()).all()
+        B.attend(t)                                        # causal: tokens 3, 4 and 5 see it
+        assert near(t, s, but(6, 3, 4, 5))
+        # (infinite keys and NaN values: a score of -inf may leave the value out)
+        assert math.isinf(k_scale) or none and torch.isnan(t["out"][3:].float()).all()
+    page, at = place(s, 70)                                # before the window of every token
+    t = {**s, "ks": s["ks"].clone(), "vs": s["vs"].clone()}
+    t["ks"][page, :, at], t["vs"][page, :, at] = math.nan, math.nan
+    B.attend(t, window=50)
+    assert near(t, s, but(6), window=50)
+
+
+@pytest.mark.parametrize("form", FAST + ["plain"])
 @pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
 def test_the_same_bits_every_time(force, form, kind):
     force(form)
