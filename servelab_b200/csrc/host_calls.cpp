@@ -275,7 +275,7 @@ PyObject* attention_args(PyObject*, PyObject* const* args, Py_ssize_t n) {
         a.scale = (float)scale;
         a.tiles = 1; a.cluster = 1;
         const bool fast = q.scalar_type() == at::kBFloat16 && (D == 64 || D == 128) && a.ldq % 8 == 0 && a.ldo % 8 == 0 &&
-                          (((uintptr_t)a.q | (uintptr_t)a.out) & 15) == 0;
+                          (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0;
         return Py_BuildValue("(NiiiOi)", as_bytes(a), device, a.T, a.S, fast ? Py_True : Py_False, kind);
     });
 }

@@ -215,8 +215,8 @@ def cache8_attention(q, k_cache, v_cache, k_scale, v_scale, out, table, cu_q, ct
     leaves it: codes of int8 or float8_e4m3fn [pages, Hkv, page size, D] and float32 scales [pages, Hkv, page size].  Request
     s has the tokens ``cu_q[s]`` .. ``cu_q[s + 1]`` - 1, its newest cached ones of ``ctx_len[s]``.  ``longest_q`` and
     ``longest_context``: what the step's plan says of the most tokens and keys of a request; launch shapes go by them,
-    results do not.  Rows behind the last request's are left as they are.  bfloat16 with head sizes 64 and 128 and rows of
-    whole 16-byte pieces: tensor cores, for cached values of up to 2^117 (int8) or 2^118; otherwise the plain kernel, float32
+    results do not.  Rows behind the last request's are left as they are.  bfloat16 with head sizes 64 and 128 and rows (queries,
+    results, caches) of whole 16-byte pieces: tensor cores, for cached values of up to 2^117 (int8) or 2^118; otherwise the plain kernel, float32
     throughout."""
     if k_scale is None or v_scale is None:
         raise L.KernelError("cache8_attention: an 8-bit cache needs its scales (tree_attention and paged_attention take others)")

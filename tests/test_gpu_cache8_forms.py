@@ -287,3 +287,18 @@ def test_the_same_bits_every_time(force, form, kind):
         s["out"].fill_(3.0)
         attend_and_check(s)
         assert torch.equal(s["out"], first)
+
+
+@pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
+@pytest.mark.parametrize("dim,tokens", [(64, 1), (128, 40)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_caches_that_begin_anywhere(kind, dim, tokens, which):
+    """A cache that is a view from an odd element on: the plain kernel takes it, as it is promised."""
+    s = B.step("bfloat16", kind, 14, 2, dim, [tokens, 2], [300, 90], 16, seed=55)
+    flat = torch.empty(s[which].numel() + 1, dtype=s[which].dtype, device=DEV)
+    view = flat[1:].view(s[which].shape)
+    view.copy_(s[which])
+    assert view.data_ptr() % 16 != 0 and view.is_contiguous()
+    attend_and_check({**s, which: view})
+    s["out"].fill_(7.0)
+    attend_and_check(s)
