@@ -54,11 +54,24 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 // Angle pos * f, reduced to [-pi, pi]: the product is exact in 64 bits, so that far positions turn as exactly as near
-// ones (in 32 bits an angle of 1e5 is off by up to 4e-3).
-__device__ __forceinline__ void turn_of(int pos, float f, float& cs, float& sn) {
+// ones (in 32 bits an angle of 1e5 is off by up to 4e-3).  Not EXACT: the product rounded to float32, the angle of the
+// models' definition and of the kernels that decode and prompt steps write their keys with (rope_cache.cu).
+template <bool EXACT> __device__ __forceinline__ void turn_of(int pos, float f, float& cs, float& sn) {
+    if constexpr (!EXACT) {
+        sincosf((float)pos * f, &sn, &cs);
+        return;
+    }
     const double a = (double)pos * (double)f;
     const double r = a - rint(a * 0.15915494309189535) * 6.283185307179586;
     sincosf((float)r, &sn, &cs);
+}
+
+// A rotation pair turned.  (Which of the products are rounded is said here, so that pairs come out as rope_cache.cu's do: in its
+// kernel for 16-byte accesses, `pieces`, and in the other one.)
+__device__ __forceinline__ void turn_pair(float& a, float& b, float cs, float sn, bool pieces) {
+    const float x = fmaf(a, cs, -__fmul_rn(b, sn));
+    b = pieces ? fmaf(b, cs, __fmul_rn(a, sn)) : fmaf(a, sn, __fmul_rn(b, cs));
+    a = x;
 }
 
 // First element of the cache rows that token t is written to, and whether it is written at all.
@@ -81,7 +94,7 @@ __device__ __forceinline__ bool token_page(const CacheWriteArgs& a, int t, int& 
 // neighbours that pass through; neighbouring lanes hold a head, so that its largest magnitude is a few shuffles (the units of
 // a head are a power of two up to 32).  A thread has one unit, whose bias it keeps, and walks tokens, the next one's elements
 // and page on their way while it works; grid (tokens at once, passes over the units).
-template <typename T, int KIND>
+template <typename T, int KIND, bool EXACT>
 __global__ void __launch_bounds__(512, 2) cache_write_vec_kernel(const CacheWriteArgs a, int units_per_head) {
     constexpr int VEC = 16 / (int)sizeof(T);
     extern __shared__ __align__(16) float trig[];          // cos[half], sin[half], of this token and the next
@@ -114,8 +127,8 @@ __global__ void __launch_bounds__(512, 2) cache_write_vec_kernel(const CacheWrit
     for (int turn = 0; t < a.T; turn ^= 1) {
         float* cs = trig + turn * 2 * half;
         float* sn = cs + half;
-        if ((int)threadIdx.x < half) turn_of(pos, freq, cs[threadIdx.x], sn[threadIdx.x]);
-        for (int i = threadIdx.x + blockDim.x; i < half; i += blockDim.x) turn_of(pos, a.inv_freq[i], cs[i], sn[i]);
+        if ((int)threadIdx.x < half) turn_of<EXACT>(pos, freq, cs[threadIdx.x], sn[threadIdx.x]);
+        for (int i = threadIdx.x + blockDim.x; i < half; i += blockDim.x) turn_of<EXACT>(pos, a.inv_freq[i], cs[i], sn[i]);
         float fa[VEC], fb[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -139,11 +152,7 @@ __global__ void __launch_bounds__(512, 2) cache_write_vec_kernel(const CacheWrit
                 const float4 s4 = *reinterpret_cast<const float4*>(sn + ea + e);
                 const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float ra = fa[e + k] * c[k] - fb[e + k] * s[k];
-                    fb[e + k] = fb[e + k] * c[k] + fa[e + k] * s[k];
-                    fa[e + k] = ra;
-                }
+                for (int k = 0; k < 4; ++k) turn_pair(fa[e + k], fb[e + k], c[k], s[k], true);
             }
         }
         float scale = 1.f, inv = 1.f;
@@ -188,8 +197,8 @@ __global__ void __launch_bounds__(512, 2) cache_write_vec_kernel(const CacheWrit
 }
 
 // The same for any even head size up to 1,024: a warp per head, element pairs over its lanes.
-template <typename T, int KIND>
-__global__ void cache_write_kernel(const CacheWriteArgs a) {
+template <typename T, int KIND, bool EXACT>
+__global__ void cache_write_kernel(const CacheWriteArgs a, bool pieces) {
     pdl_launch_dependents();
     pdl_wait();
     constexpr int MOST = 16;                               // pairs a lane holds
@@ -216,10 +225,8 @@ __global__ void cache_write_kernel(const CacheWriteArgs a) {
             if (a.bias) { fa[n] += a.bias[off + ea]; fb[n] += a.bias[off + eb]; }
             if (rot) {
                 float cs, sn;
-                turn_of(pos, a.inv_freq[i], cs, sn);
-                const float ra = fa[n] * cs - fb[n] * sn;
-                fb[n] = fb[n] * cs + fa[n] * sn;
-                fa[n] = ra;
+                turn_of<EXACT>(pos, a.inv_freq[i], cs, sn);
+                turn_pair(fa[n], fb[n], cs, sn, pieces);
             }
             amax = max_nan(amax, max_nan(fabsf(fa[n]), fabsf(fb[n])));
         }
@@ -252,23 +259,26 @@ __global__ void cache_write_kernel(const CacheWriteArgs a) {
     }
 }
 
-template <typename T, int KIND>
-int launch_cache_write(const CacheWriteArgs& a, cudaStream_t st) {
+template <typename T, int KIND, bool EXACT>
+int launch_cache_write_turned(const CacheWriteArgs& a, cudaStream_t st) {
     constexpr int VEC = 16 / (int)sizeof(T);
     const int rot = a.inv_freq != nullptr ? a.rot : 0;
     const int per_head = a.D / (2 * VEC);
-    const bool vec_ok = a.D % (2 * VEC) == 0 && per_head <= 32 && (per_head & (per_head - 1)) == 0 && rot % (2 * VEC) == 0 &&
-                        a.ld % VEC == 0 && a.ldq % VEC == 0 &&
-                        ((uintptr_t)a.qkv | (uintptr_t)a.q_out | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.bias) % 16 == 0;
+    const bool pieces = a.D % (2 * VEC) == 0 && rot % (2 * VEC) == 0 && a.ld % VEC == 0 && a.ldq % VEC == 0 &&
+                        ((uintptr_t)a.qkv | (uintptr_t)a.q_out | (uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0;
+    const bool vec_ok = pieces && per_head <= 32 && (per_head & (per_head - 1)) == 0 && (uintptr_t)a.bias % 16 == 0;
     const int heads = a.H + 2 * a.Hkv;
-    if (!vec_ok) return slb_launch(cache_write_kernel<T, KIND>, dim3(a.T), dim3(32 * (heads < 8 ? heads : 8)), 0, st, a);
+    if (!vec_ok) return slb_launch(cache_write_kernel<T, KIND, EXACT>, dim3(a.T), dim3(32 * (heads < 8 ? heads : 8)), 0, st, a, pieces);
     const int units = heads * per_head;
     const int passes = (units + 511) / 512;
     const int threads = ((units + passes - 1) / passes + 31) / 32 * 32;      // (whole heads: 32 is a multiple of per_head)
     // as many blocks as the SMs hold (64 registers a thread): every block has a token at least
     const int at_once = slb_num_sms() * (1024 / threads);
-    return slb_launch(cache_write_vec_kernel<T, KIND>, dim3(a.T < at_once ? a.T : at_once, passes), dim3(threads),
+    return slb_launch(cache_write_vec_kernel<T, KIND, EXACT>, dim3(a.T < at_once ? a.T : at_once, passes), dim3(threads),
                       (size_t)rot * 2 * sizeof(float), st, a, per_head);
+}
+template <typename T, int KIND> int launch_cache_write(const CacheWriteArgs& a, cudaStream_t st) {
+    return a.exact ? launch_cache_write_turned<T, KIND, true>(a, st) : launch_cache_write_turned<T, KIND, false>(a, st);
 }
 
 // ------------------------------------------------------------------------------------------------ reading back

@@ -13,6 +13,7 @@ struct CacheWriteArgs {
     void* q_out; long long ldq;
     void* k; void* v; float* ks; float* vs;
     int T, H, Hkv, D, kind;
+    int exact;                                   // angles in 64 bits; 0: rounded to float32, as the other writers' are
 };
 struct CacheReadArgs {
     const void* k; const void* v; const float* ks; const float* vs;

@@ -144,10 +144,10 @@ template <typename A> A from_bytes(PyObject* o) {
 }
 
 // write_args(what, qkv, bias, positions, slots, seq_of_token, block_table, page size, inv_freq, rotary_dim, q_out, k_cache, v_cache,
-// k_scale, v_scale, heads, kv heads, head size) -> (structure, device)
+// k_scale, v_scale, heads, kv heads, head size, angles in 64 bits) -> (structure, device)
 PyObject* write_args(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return guarded(args, n, [&]() -> PyObject* {
-        Arguments in(args, n, 18);
+        Arguments in(args, n, 19);
         in.text();
         const at::Tensor &qkv = in.tensor("qkv"), *bias = in.tensor_or_none("bias"), &pos = in.tensor("positions"),
                          *slots = in.tensor_or_none("slots"), &seq = in.tensor("seq_of_token"), &table = in.tensor("block_table");
@@ -156,7 +156,7 @@ PyObject* write_args(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int rot = in.size("rotary size");
         const at::Tensor &q_out = in.tensor("q_out"), &k = in.tensor("k_cache"), &v = in.tensor("v_cache"),
                          *ks = in.tensor_or_none("k_scale"), *vs = in.tensor_or_none("v_scale");
-        const int H = in.size("heads"), Hkv = in.size("kv heads"), D = in.size("head size");
+        const int H = in.size("heads"), Hkv = in.size("kv heads"), D = in.size("head size"), exact = in.size("exact_angles");
         check_rows(qkv, "qkv");
         const int kind = cache_kind(qkv, k, v, ks, vs, Hkv, page, D);
         const int64_t width = ((int64_t)H + 2 * (int64_t)Hkv) * D;
@@ -186,7 +186,7 @@ PyObject* write_args(PyObject*, PyObject* const* args, Py_ssize_t n) {
         a.inv_freq = address<float>(inv_freq); a.rot = inv_freq != nullptr ? rot : 0;
         a.q_out = address<void>(q_out); a.ldq = q_out.stride(0);
         a.k = address<void>(k); a.v = address<void>(v); a.ks = address<float>(ks); a.vs = address<float>(vs);
-        a.T = in_int(T, "tokens"); a.H = H; a.Hkv = Hkv; a.D = D; a.kind = kind;
+        a.T = in_int(T, "tokens"); a.H = H; a.Hkv = Hkv; a.D = D; a.kind = kind; a.exact = exact != 0;
         return Py_BuildValue("(Ni)", as_bytes(a), device);
     });
 }

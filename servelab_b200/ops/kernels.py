@@ -2051,16 +2051,18 @@ def cache_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], positions: torc
                 seq_of_token: torch.Tensor, block_table: torch.Tensor, page_size: int, inv_freq: Optional[torch.Tensor],
                 rotary_dim: int, q_out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                 k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor], num_heads: int, num_kv_heads: int,
-                head_dim: int) -> None:
+                head_dim: int, exact_angles: bool = True) -> None:
     """``qkv_rope_cache`` for caches in 8 bits and for drafted tokens: adds ``bias`` (float32), rotates queries and keys by
     ``positions``, stores the queries in ``q_out`` [T, H D] and writes keys and values to the pages at ``slots`` (None: at
     their positions; tokens of a tree share positions, never slots).  Caches of int8 or float8_e4m3fn take codes and, per
     (token, kv head), the scale max |x| / 127 or / 448 (at least 2^-126); a row with an infinity or NaN gets the scale NaN.
     Caches of the rows' type take the rows (``k_scale`` and ``v_scale`` None).  Tokens without a page are not written; no
-    two tokens may have one slot."""
+    two tokens may have one slot.  ``exact_angles``: position times frequency in 64 bits, so that far positions turn as exactly as
+    near ones; False: rounded to float32, the angles that ``qkv_rope_cache`` and the fused products turn by (at position 30,000 up
+    to 2e-3 away), for a cache whose other rows they write."""
     host = L.host()
     args, device = host.write_args("cache_write", qkv, bias, positions, slots, seq_of_token, block_table, page_size, inv_freq, rotary_dim,
-                                   q_out, k_cache, v_cache, k_scale, v_scale, num_heads, num_kv_heads, head_dim)
+                                   q_out, k_cache, v_cache, k_scale, v_scale, num_heads, num_kv_heads, head_dim, exact_angles)
     entry = L.entry(L.core(), "slb_cache_write_f32" if qkv.dtype is _F32 else "slb_cache_write_bf16")
     L.check(host.launch("cache_write", entry, args, _current_stream("cache_write", device)), "cache_write")
 

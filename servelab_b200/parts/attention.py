@@ -116,9 +116,10 @@ class PagedAttention(Mixer):
         return linear(out, self.w_o, self.b_o, consumer="norm")
 
     def _write(self, ctx, qkv, bias, cache, table, inv_freq, rotary_dim, q):
+        # (one rotation for all steps: drafts share their cache with what decode and prompt steps wrote)
         s = self.spec
         K.cache_write(qkv, bias, ctx.positions, ctx.slots, ctx.seq_of_token, table, cache.page_size, inv_freq, rotary_dim, q,
-                      cache.k, cache.v, cache.k_scale, cache.v_scale, s.num_heads, s.num_kv_heads, s.head_dim)
+                      cache.k, cache.v, cache.k_scale, cache.v_scale, s.num_heads, s.num_kv_heads, s.head_dim, exact_angles=False)
 
     def _attend(self, ctx, q, cache, table, out):
         s = self.spec

@@ -203,3 +203,34 @@ def test_generation_with_and_without_graphs(model, dtype, kv):
     assert eng.runner.graph_replays > 0 and eng.runner.portion_graph_replays > 0
     assert eng.runner.storage.layer_caches[0].k.dtype == KINDS[kv]
     assert got == tokens(cuda_graphs=False)[0]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("kv", ["auto", "int8"])
+def test_far_drafts_leave_the_keys_that_decoding_leaves(model, dtype, kv):
+    """The first layer's keys and values at slots around 30,000 (they go by token and position alone), written by a step of
+    single tokens, by a portion of a prompt and by a tree that is a chain: the very same rows."""
+    start, n = 30001, 5
+    ids = H.random_ids(n, model["cfg"]["vocab_size"], 77)
+    sess = session(model, dtype, kv, poison=False, pages=-(-(start + 64) // model["page"]))
+    runner = sess.runner
+    written = {}
+    for how in ("single", "portion", "tree"):
+        assert runner.cache.open(how)
+        assert runner.cache.ensure(how, start + n)
+        if how == "single":
+            for j in range(n):
+                runner.step([runner.entry(how, ids[j:j + 1], start + j, [0])])
+        else:
+            runner.step([runner.entry(how, ids, start, [n - 1], list(range(-1, n - 1)) if how == "tree" else None)])
+        written[how] = runner.cached_rows(how, n, start=start)
+        runner.cache.release(how)
+    for how in ("portion", "tree"):
+        for a, b in zip(written[how], written["single"]):
+            # (float32 products do not depend on the step; bfloat16 steps of few tokens rotate before they round, and the products
+            # of different sizes add up in different orders: two roundings apart, or a code)
+            if dtype == "float32":
+                assert torch.equal(a, b), how
+            else:
+                top = b.float().abs().amax(-1, keepdim=True)
+                assert ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + (2.0 ** -6 if kv == "int8" else 2.0 ** -8) * top).all(), how

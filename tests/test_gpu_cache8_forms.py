@@ -302,3 +302,28 @@ def test_caches_that_begin_anywhere(kind, dim, tokens, which):
     attend_and_check({**s, which: view})
     s["out"].fill_(7.0)
     attend_and_check(s)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("heads,kv,dim,rotary", [(14, 2, 64, 64), (4, 2, 128, 64), (5, 5, 20, 12), (4, 2, 48, 48)])
+def test_rows_with_the_angles_of_other_writers(dtype, heads, kv, dim, rotary):
+    """``cache_write`` without exact angles leaves what ``qkv_rope_cache`` leaves, at any position; and with codes what rows that
+    it has turned (exactly, in float32) become as codes."""
+    w = B.write_case(dtype, "plain", heads, kv, dim, rotary, [7, 33], [130001, 30000], 16, seed=dim)
+    other = {n: torch.zeros_like(w[n]) for n in ("q_out", "k", "v")}
+    args = (w["qkv"], w["bias"], w["positions"])
+    B.K().qkv_rope_cache(*args, w["seq"], w["table"], 16, w["inv"], rotary, other["q_out"], other["k"], other["v"], heads, kv, dim)
+    B.K().cache_write(*args, None, w["seq"], w["table"], 16, w["inv"], rotary, w["q_out"], w["k"], w["v"], None, None, heads, kv, dim,
+                      exact_angles=False)
+    for n in other:
+        assert torch.equal(w[n], other[n]), n
+    if dtype == "float32":
+        codes = [torch.zeros(w["k"].shape, dtype=torch.int8, device=DEV) for _ in range(2)]
+        scales = [torch.zeros(w["k"].shape[:3], device=DEV) for _ in range(2)]
+        B.K().cache_write(*args, None, w["seq"], w["table"], 16, w["inv"], rotary, w["q_out"], *codes, *scales, heads, kv, dim,
+                          exact_angles=False)
+        for rows, code, scale in zip((w["k"], w["v"]), codes, scales):
+            want = rows.abs().amax(-1) / 127               # (a product with 1 / 127 or a division: a unit apart at most)
+            assert ((scale - want).abs() <= 2.0 ** -22 * want)[want > 0].all()
+            # half a code, and what the scale's reciprocal and the product round
+            assert ((code * scale[..., None] - rows).abs() <= (0.5 + 2.0 ** -14) * scale[..., None]).all()
