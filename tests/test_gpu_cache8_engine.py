@@ -234,3 +234,24 @@ def test_far_drafts_leave_the_keys_that_decoding_leaves(model, dtype, kv):
             else:
                 top = b.float().abs().amax(-1, keepdim=True)
                 assert ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + (2.0 ** -6 if kv == "int8" else 2.0 ** -8) * top).all(), how
+
+
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+@pytest.mark.parametrize("name", ["D", "E"])
+def test_replayed_steps_planned_for_long_contexts(name, kv, tmp_path):
+    """Decode steps replay a graph whose launches were chosen for 32,768 keys (head sizes 64 and 128): logits near those of steps
+    that are planned for their own contexts, which are short."""
+    cfg, seed, page = H.CONFIGS[name]
+    long = {"name": name, "cfg": {**cfg, "max_position_embeddings": 32768}, "folder": str(tmp_path), "page": page}
+    H.make_model(long["folder"], long["cfg"], seed, std_of=H.STD_OF.get(name))
+    requests = {f"r{i}": H.random_ids(n, cfg["vocab_size"], 80 + i) for i, n in enumerate([70, 33, 58])}
+    steps = H.trace_bulk_tail(requests, tail=12)
+    got = {}
+    for graphs in (True, False):
+        sess = session(long, "bfloat16", kv, pages=32768 // page + 4, cuda_graphs=graphs)
+        assert sess.runner.max_model_len == 32768
+        got[graphs] = H.collect(steps, H.run_session(sess, steps), cfg["vocab_size"])
+        assert (sess.runner.graph_replays > 0) == graphs
+    # (two sums in other orders of the same codes: roundings of bfloat16, as the bounds of a cache in that type)
+    far = max(float(np.abs(row - got[False][r][j]).max()) for r in requests for j, row in got[True][r].items())
+    assert far <= TOL["bfloat16"][name]
