@@ -9,7 +9,7 @@
 //                  O += P.V    (M=128 N=D,  K=16 x 4)                                             -> pv_done
 //   softmax warps  32 rows each: 64 scores times their keys' scales, running maximum and sum in float32, probabilities times
 //                  the values' scales in 16 bits back to tensor memory; four rows a lane where all keys are seen, a row a
-//                  lane and a mask where not                                                      -> p_full
+//                  lane and a mask where not, where scores are huge or query rows have factors of their own   -> p_full
 //
 // A scout warp runs ahead of the loaders: it looks pages up, asks for their rows and brings the scales.
 // Scores are double buffered.  A barrier is one of a pair indexed by the tile's parity.  The running maximum is only raised
@@ -19,9 +19,12 @@
 // Few tiles leave SMs idle: then blocks (`parts`, or one more) share a tile's keys and a second kernel adds their results up.
 // (Through the shared memory of a cluster of eight that took 7,500 cycles a block, and clusters left half of the SMs' places empty.)
 //
-// What bounds it: the chain of the roles.  A tile takes 3,700 cycles with two blocks an SM, whose issue slots are busy to 48 % and
-// tensor pipe to 23 %; a block's start (tile, pages, queries, first keys) takes 7,500.  28 heads over 4 of 128: two portions of 257
-// tokens over 2,043 keys in int8 40.0 us, eight trees of 32 drafts over 2,040 keys 27.6, one of 64 over 16,380 keys in bfloat16 31.4.
+// What bounds it: the chain of the roles.  A tile takes 3,700 cycles with two blocks an SM, whose issue slots are busy to 53 % and
+// tensor pipe to 24 %; a block's start (tile, pages, queries, first keys) takes 7,500.  28 heads over 4 of 128: two portions of 257
+// tokens over 2,043 keys in int8 40.2 us, eight trees of 32 drafts over 2,040 keys 28.2, one of 64 over 16,380 keys in bfloat16 32.4.
+//
+// Over a bfloat16 cache probabilities are rounded to bfloat16 (both operands of a product have one type): at most 2^-8 of a weight;
+// the last case is 2.3e-3 of its results' size away from 64 bits, where rounding the results alone makes 1.7e-3.
 //
 // Every wait is bounded; a role that gives up sets the status word and leaves its loop, the block frees its tensor memory
 // and has no result (its part: NaN).

@@ -2085,7 +2085,8 @@ def _few_resident(head_dim: int, kind: int, block: int, cluster: int) -> int:
 
 
 def cache_few_shares(units: int, slices: int, block: int, resident) -> "tuple[int, int, int]":
-    """(parts, blocks of a cluster, cost) that share the keys of a tile of ``block`` rows, 8 (two blocks an SM) or 16 (one);
+    """(parts, blocks of a cluster, cost) that share the keys of a tile of ``block`` rows, 8 (counted as two blocks an SM; over a
+    bfloat16 cache with head size 128, whose rings take 201 KB, it is one, of which only the rounds know) or 16 (one);
     ``resident(cluster)``: clusters that the device holds at once.  An SM that has n blocks of a launch takes the
     time of their slices of 16 keys (a tenth less with two blocks at a time) and, for every round of blocks, that of 25 slices before
     and behind them; a cluster adds 3 to 6, parts behind clusters of eight (a second kernel) 30 and 10 a part.  us with clusters
