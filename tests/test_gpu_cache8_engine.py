@@ -255,3 +255,52 @@ def test_replayed_steps_planned_for_long_contexts(name, kv, tmp_path):
     # (two sums in other orders of the same codes: roundings of bfloat16, as the bounds of a cache in that type)
     far = max(float(np.abs(row - got[False][r][j]).max()) for r in requests for j, row in got[True][r].items())
     assert far <= TOL["bfloat16"][name]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+@pytest.mark.parametrize("far", [0, 4000])
+def test_mixer_that_reads_anothers_8_bit_cache(dtype, kv, far):
+    """A run without a cache of its own: its queries over the rows that another run left, also at far positions."""
+    from servelab_b200.config import AttentionSpec, RotarySpec
+    from servelab_b200.engine.batch import BatchEntry, StepContext
+    from servelab_b200.ops import kernels as K
+    from servelab_b200.parts import MIXERS, BuildEnv, LayerCache, build_part, part_class
+    from servelab_b200.weights import RandomSource, WeightStore
+    heads, kvh, hid, T, ps, dim = 6, 2, 40, 21, 16, 64
+    spec = AttentionSpec(hidden_size=hid, num_heads=heads, num_kv_heads=kvh, head_dim=dim, qkv_bias=True, out_bias=False, window=T,
+                         position=RotarySpec(head_dim=dim, rotary_dim=dim, theta=1e4))
+    decls = part_class(MIXERS, spec).declare(spec, "a")
+    parts, weights = [], []
+    for seed in (3, 4):
+        src = RandomSource(decls, seed, std=0.08, dtype=DT[dtype])
+        parts.append(build_part(MIXERS, spec, "a", BuildEnv(device=DEV, dtype=DT[dtype], page_size=ps)))
+        parts[-1].load(WeightStore(src, decls, DT[dtype], DEV))
+        weights.append({d.name: src.read(d.name).double() for d in decls})
+    torch.manual_seed(6)
+    x = torch.randn(T, hid).to(DT[dtype])
+    first = far // ps
+    pages = [-1] * first + [3, 0, 2]
+    codes = torch.zeros((2, 4, kvh, ps, dim), dtype=torch.uint8, device=DEV).view(KINDS[kv])
+    scales = torch.zeros((2, 4, kvh, ps), device=DEV)
+    cache = LayerCache(group=0, k=codes[0], v=codes[1], page_size=ps, k_scale=scales[0], v_scale=scales[1])
+    ctx = StepContext.pack([BatchEntry([0] * T, first * ps, (), [pages])], 1, DEV)
+    parts[0].forward(ctx, x.to(DEV), cache, True)
+    before = [t.clone() for t in (codes.view(torch.uint8), scales)]
+    got = K.plain_unless(None, parts[1].forward(ctx, x.to(DEV), cache, False)).double().cpu()
+    assert torch.equal(codes.view(torch.uint8), before[0]) and torch.equal(scales, before[1])
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=DEV)
+    kc, vc = torch.empty(T, kvh, dim, device=DEV), torch.empty(T, kvh, dim, device=DEV)
+    K.cache_read(cache.k, cache.v, cache.k_scale, cache.v_scale, i32([pages]), i32([first * ps]), i32([0, T]), ps, kc, vc)
+    w = weights[1]
+    q = P.linear(x.double(), w["a.q_proj.weight"], w["a.q_proj.bias"]).view(T, heads, dim)
+    # angles are float32 products of position and frequency, by definition
+    angle = (torch.arange(first * ps, first * ps + T).float()[:, None] * P.rope_inv_freq(dim, 1e4).float()[None]).double()
+    a, b = q[..., :dim // 2], q[..., dim // 2:]
+    q = torch.cat([a * angle.cos()[:, None] - b * angle.sin()[:, None], b * angle.cos()[:, None] + a * angle.sin()[:, None]], -1)
+    # (far on, slots of the window before the first token have no page: keys and values of zeros, which count)
+    zeros = T if far else 0
+    kc, vc = (torch.cat([torch.zeros(zeros, kvh, dim), t.cpu()]).double() for t in (kc, vc))
+    q = torch.cat([torch.zeros(zeros, heads, dim).double(), q])
+    want = P.linear(P.causal_attention(q, kc, vc, T).double()[zeros:], w["a.o_proj.weight"])
+    assert (got - want).abs().max() <= {"float32": 1e-5, "bfloat16": 2e-2}[dtype]

@@ -327,3 +327,21 @@ def test_rows_with_the_angles_of_other_writers(dtype, heads, kv, dim, rotary):
             assert ((scale - want).abs() <= 2.0 ** -22 * want)[want > 0].all()
             # half a code, and what the scale's reciprocal and the product round
             assert ((code * scale[..., None] - rows).abs() <= (0.5 + 2.0 ** -14) * scale[..., None]).all()
+
+
+@pytest.mark.parametrize("form", FAST + ["plain"])
+@pytest.mark.parametrize("kind", ["plain", "int8"])
+@pytest.mark.parametrize("window", [0, 90])
+def test_a_tree_beside_a_long_portion(force, form, kind, window):
+    """A portion of 331 tokens as a chain and a tree of 37 drafts in one step: eleven words of a mask."""
+    from servelab_b200.engine.batch import tree_depths, tree_mask
+    force(form)
+    q_lens, ctxs = [331, 37, 1], [400, 200, 90]
+    trees = [range(-1, 330), B.parents_of(37, 5), [-1]]
+    s = B.step("bfloat16", kind, 4, 2, 64, q_lens, ctxs, 16, seed=56, pad=2)
+    words = tree_mask(trees)
+    bits = [sum((int(w) & 0xFFFFFFFF) << 32 * i for i, w in enumerate(row)) for row in words]
+    positions = [c - n + d for n, c, t in zip(q_lens, ctxs, trees) for d in tree_depths(t)]
+    mask = torch.cat([torch.from_numpy(words).to(DEV), torch.full((2, words.shape[1]), -1, dtype=torch.int32, device=DEV)])
+    B.attend(s, window=window, mask=mask, positions=C.i32(positions + [0, 0], DEV))
+    B.check(s, window=window, bits=bits, positions=positions)
