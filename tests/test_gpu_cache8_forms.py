@@ -139,8 +139,7 @@ def test_value_scales_near_the_largest_that_count(force, form, kind):
 
 @pytest.mark.parametrize("form", FAST + ["plain"])
 @pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
-@pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("window", [0, 1, 20, 130])
+@pytest.mark.parametrize("dim,window", [(64, 0), (128, 0), (128, 1), (64, 20), (128, 130)])
 def test_portions_and_windows(force, form, kind, dim, window):
     calls = force(form)
     s = B.step("bfloat16", kind, 14, 2, dim, [5, 0, 33, 1, 70], [5, 0, 200, 77, 331], 16, seed=47, pad=1)
@@ -180,8 +179,7 @@ def one_takes_all(s, q):
 
 @pytest.mark.parametrize("form", FAST + ["plain"])
 @pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
-@pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("far", [18, 22, 24, 25, 26, 27, 28, 30, 34, 60])
+@pytest.mark.parametrize("dim,far", [(64, 18), (128, 22), (64, 24), (128, 25), (64, 26), (128, 27), (64, 28), (128, 30), (64, 34), (128, 60)])
 def test_scores_of_any_size(force, form, kind, dim, far):
     """Scores of about 2^far, also where all of them are negative: numbers throughout, and one key's value where float32 tells
     which; for value scales of different sizes."""
@@ -202,8 +200,7 @@ def test_scores_of_any_size(force, form, kind, dim, far):
 
 @pytest.mark.parametrize("form", FAST)
 @pytest.mark.parametrize("kind", ["plain", "int8", "e4m3"])
-@pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("far", [14, 16, 17, 20, 34, 60, 100])
+@pytest.mark.parametrize("dim,far", [(64, 14), (128, 16), (64, 17), (128, 20), (64, 34), (128, 34), (64, 60), (128, 100)])
 def test_query_rows_of_very_different_size(force, form, kind, dim, far):
     """Tokens and heads whose queries are 2^far times their neighbours', above or below."""
     force(form)
@@ -283,9 +280,13 @@ def test_the_same_bits_every_time(force, form, kind):
     s = B.step("bfloat16", kind, 14, 2, 128, [40, 1], [1500, 700], 16, seed=53)
     attend_and_check(s)
     first = s["out"].clone()
-    for _ in range(5):
+    mask, positions, _, _ = chain(s)
+    for _ in range(20):
         s["out"].fill_(3.0)
-        attend_and_check(s)
+        if kind == "plain":
+            B.attend(s, mask=mask, positions=positions)
+        else:
+            B.attend(s)
         assert torch.equal(s["out"], first)
 
 
