@@ -495,6 +495,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) plain_cache_attention_kernel
     const bool vec = D % PIECE == 0 && (uintptr_t)kbase % 16 == 0;
     for (int tile = blockIdx.y / a.Hkv; (long long)tile * PA_ROWS < (long long)q_len * g; tile += a.tiles) {
         const int row0 = tile * PA_ROWS, nrows = min(PA_ROWS, q_len * g - row0);
+        bool far = false;                                  // an element is so large that sums with codes may overflow
         __syncthreads();
         for (int i = threadIdx.x; i < PA_ROWS * 32 * DL; i += blockDim.x) {
             const int r = i / (32 * DL), d = i - r * (32 * DL);
@@ -504,8 +505,16 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) plain_cache_attention_kernel
                 x = to_float(reinterpret_cast<const T*>(a.q)[(size_t)tok * a.ldq + (size_t)h * D + d]);
             }
             qs[r][d] = x;
+            far |= fabsf(x) > 1.2379400392853803e27f;      // 2^90
         }
-        __syncthreads();
+        float moved = 1.f;
+        if (KIND == CACHE_PLAIN) {
+            __syncthreads();
+        } else if (__syncthreads_or(far)) {                // (their keys' scales are as small: 2^40 moves there)
+            for (int i = threadIdx.x; i < PA_ROWS * 32 * DL; i += blockDim.x) qs[i / (32 * DL)][i % (32 * DL)] *= 9.094947017729282e-13f;
+            moved = 1099511627776.f;
+            __syncthreads();
+        }
         RowView view[PA_ROWS];
         int least = ctx;                                   // first slot that a row of the tile sees
 #pragma unroll
@@ -576,7 +585,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) plain_cache_attention_kernel
                     }
                 }
                 float kscale = a.scale * 1.4426950408889634f;
-                if constexpr (KIND != CACHE_PLAIN) { kscale *= a.ks[row]; vscale = a.vs[row]; }
+                if constexpr (KIND != CACHE_PLAIN) { kscale = kscale * moved * a.ks[row]; vscale = a.vs[row]; }
 #pragma unroll
                 for (int r = 0; r < PA_ROWS; ++r) sc[r] = __fmul_rn(sc[r], kscale);   // (the maximum and the exponents go by this number)
             }

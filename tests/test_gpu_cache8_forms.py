@@ -114,7 +114,7 @@ def test_a_key_that_takes_all_weight_and_has_no_value(force, form, kind, dim, sl
     assert calls == [FORMS[form][0]]
 
 
-@pytest.mark.parametrize("form", FAST)
+@pytest.mark.parametrize("form", FAST + ["plain"])
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
 def test_value_scales_over_forty_powers_of_two(force, form, kind):
     calls = force(form)
@@ -122,7 +122,7 @@ def test_value_scales_over_forty_powers_of_two(force, form, kind):
     s["vs"] *= torch.exp2(torch.randint(-20, 21, s["vs"].shape, generator=B.gen(44), device=DEV).float())
     for factor in (1.0, 2.0 ** 80, 2.0 ** -90):
         attend_and_check({**s, "vs": s["vs"] * factor})
-    for factor in (2.0 ** 60, 2.0 ** -60, 2.0 ** 120):
+    for factor in (2.0 ** 60, 2.0 ** -60, 2.0 ** 120, 2.0 ** 125):
         attend_and_check({**s, "q": (s["q"].float() * factor).to(torch.bfloat16), "ks": s["ks"] / factor})
     assert set(calls) == {FORMS[form][0]}
 
